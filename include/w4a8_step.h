@@ -78,7 +78,9 @@ int w4a8_rope_append(const float *qkv, int heads, const w4a8_kv_cache *cache, co
  * aligned, out no part of q. Scores, softmax and sums are float32; q and p meet
  * the cache's 16-bit values split into as many 16-bit parts as hold 22 bits or
  * more of them. A row without a position left (empty, or all its pages absent)
- * gives zeros. Infinite K or V at a position attended gives non-finite outputs.
+ * gives zeros. Finite K and V give finite outputs, V up to the type's largest
+ * included (for which bf16 weights under 2^-88 of a row's largest are dropped).
+ * Infinite K or V at a position attended gives non-finite outputs.
  * workspace: w4a8_paged_attention_workspace_bytes of device memory, 16-byte
  * aligned, its contents without meaning between calls; calls that may overlap
  * need one each. */

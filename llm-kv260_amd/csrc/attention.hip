@@ -41,9 +41,7 @@ constexpr int TILE = 32;          // positions a wave takes at a time
 constexpr int WAVES = 4;
 constexpr int HEADS = 16;         // columns: query heads a workgroup takes, of a row or of several
 constexpr int MAX_SPLITS = 256;   // of a row: the join gives each a thread
-// p is held relative to ref - P_SHIFT, at most 2^(P_SHIFT + P_LAZY): below
-// fp16's largest, and its low part's 2^-25 stays under 2^-32 of the largest p.
-constexpr float P_SHIFT = 7.0f, P_LAZY = 8.0f;
+constexpr float P_LAZY = 8.0f;    // scores may pass ref by it before ref moves
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -58,6 +56,9 @@ struct Half<f16_t> {
     static constexpr int PARTS = 2;
     static constexpr uint32_t EXPONENT = 0x7C00;
     static constexpr bool SCALED = true;    // q is brought to fp16's range by a power of two a head
+    // log2 of what stands for a p of 1 at ref: 2^(7 + P_LAZY) is below fp16's largest, and the low part's 2^-25 under
+    // 2^-32 of the largest p.
+    static __device__ __forceinline__ float unit(int) { return 7.0f; }
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -68,6 +69,11 @@ struct Half<bf16_t> {
     static constexpr int PARTS = 3;
     static constexpr uint32_t EXPONENT = 0x7F80;
     static constexpr bool SCALED = false;
+    // V may be as large as a float32: p is at most 1 / len, so that no sum of p v passes the largest v. What is left of
+    // float32's range below holds p to 22 bits down to 2^-64 of the row's largest, and none under 2^-88 (len = 2^30).
+    static __device__ __forceinline__ float unit(int len) {
+        return -P_LAZY - (float)(len > 1 ? 32 - __builtin_clz((unsigned)(len - 1)) : 0);
+    }
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -189,9 +195,11 @@ struct Query {
     }
 };
 
-// Positions: the lane's column's own, and the least and most of the workgroup's.
+// Positions: the lane's column's own, and the least and most of the workgroup's; Half::unit of the most, which all splits
+// of a row share.
 struct Lens {
     int own, least, most;
+    float unit;
 };
 
 template <class T, int D>
@@ -261,7 +269,7 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) st.o[i] *= alpha;
     }
-    const float base = st.ref == -INFINITY ? 0.0f : st.ref - P_SHIFT;
+    const float base = st.ref == -INFINITY ? 0.0f : st.ref - len.unit;
 #pragma unroll
     for (int j = 0; j < 8; ++j) s[j] = __builtin_amdgcn_exp2f(s[j] - base);
     st.sum += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
@@ -340,6 +348,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_kernel(AttendArgs a) {
     } else {
         len.own = len.least = len.most = kv_len(a.pos[row], a.table_pages, a.page_shift);
     }
+    len.unit = H::unit(len.most);
     const int used = splits_used(len.most, a.splits);
     if (split >= used && split > 0) return;
     const int end = (len.most + TILE - 1) / TILE;
