@@ -209,7 +209,7 @@ struct State {
 };
 
 template <class T, int D, bool ROWS>
-__device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, int first, Lens len, int lane, int group,
+__device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, int first, Lens len, int lane,
                                             State<T, D> &st) {
     using H = Half<T>;
     const int g = lane >> 4;
@@ -229,7 +229,13 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
     for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[4 * h + r] = H::SCALED ? __builtin_amdgcn_ldexpf(acc[h][r], q.exp) : acc[h][r];
-    bool apart = false;
+    // Dimension n D / 16 + i of the lane's eight positions.
+    const auto operand = [&](int i) {
+        const auto word = [&](int j) { return t.v[j][i / 8][(i % 8) / 2]; };
+        const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+        return make_uint4(__builtin_amdgcn_perm(word(1), word(0), sel), __builtin_amdgcn_perm(word(3), word(2), sel),
+                          __builtin_amdgcn_perm(word(5), word(4), sel), __builtin_amdgcn_perm(word(7), word(6), sel));
+    };
     if (t.page[0] < 0 || t.page[1] < 0 || first + TILE > len.least) {
         // Masked positions: no score, and zeros for V where no row has stored any, whose bits may be anything.
 #pragma unroll
@@ -243,17 +249,38 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
                     for (int i = 0; i < Tile<D>::V_LOADS; ++i) t.v[4 * h + r][i] = 0;
             }
         // A position that one row attends and another does not holds the first one's V: where that is no number, its
-        // product with the other's p of 0 is none either, and the rows go one at a time.
+        // product with the other's p of 0 is none either. It is taken out, and the outputs that it belongs to are none:
+        // a product of its places with the columns that attend them tells which.
         if constexpr (ROWS) {
-            bool odd = false;
+            // Bits 0 and 16: whether a word's halves are infinite or NaN, their exponents all ones.
+            const auto odd = [&](uint32_t w) {
+                constexpr uint32_t e = H::EXPONENT * 0x10001u, unit = (0x8000u - H::EXPONENT) * 0x10001u;
+                return ((w & e) + unit) >> 15 & 0x10001u;
+            };
+            uint32_t any = 0;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) {
-                    const uint32_t w = t.v[j][i / 4][i % 4], e = Half<T>::EXPONENT;
-                    odd |= (w & e) == e || (w >> 16 & e) == e;
+                for (int i = 0; i < D / 32; ++i) any |= odd(t.v[j][i / 4][i % 4]);
+            if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
+                typename H::vec seen;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) seen[j] = (T)(first + 16 * (j / 4) + 4 * g + j % 4 < len.own ? 1.0f : 0.0f);
+                const uint32_t one = __builtin_bit_cast(uint16_t, (T)1.0f);
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint4 v = operand(i);
+                    const uint4 at = make_uint4(odd(v.x) * one, odd(v.y) * one, odd(v.z) * one, odd(v.w) * one);
+                    const f32x4 some = H::mfma(__builtin_bit_cast(typename H::vec, at), seen, f32x4{});
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) st.o[i][r] = some[r] > 0.0f ? NAN : st.o[i][r];
+                    __builtin_amdgcn_sched_barrier(0);      // one at a time: this is rare, and its registers are not to be had
                 }
-            apart = __builtin_amdgcn_ballot_w64(odd) != 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) t.v[j][i / 4][i % 4] &= ~(odd(t.v[j][i / 4][i % 4]) * 0xFFFFu);
+            }
         }
     }
     float top = s[0];
@@ -275,38 +302,11 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
     st.sum += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     typename H::vec p[H::PARTS];
     split8<T>(s, p);
-    // Dimension n D / 16 + i of the lane's eight positions.
-    const auto operand = [&](int i) {
-        const auto word = [&](int j) { return t.v[j][i / 8][(i % 8) / 2]; };
-        const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
-        return make_uint4(__builtin_amdgcn_perm(word(1), word(0), sel), __builtin_amdgcn_perm(word(3), word(2), sel),
-                          __builtin_amdgcn_perm(word(5), word(4), sel), __builtin_amdgcn_perm(word(7), word(6), sel));
-    };
-    const auto add = [&](uint4 v, f32x4 o) {
 #pragma unroll
-        for (int b = 0; b < H::PARTS; ++b) o = H::mfma(__builtin_bit_cast(typename H::vec, v), p[b], o);
-        return o;
-    };
-    if (!ROWS || !apart) {
+    for (int i = 0; i < D / 16; ++i) {
+        const uint4 v = operand(i);
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) st.o[i] = add(operand(i), st.o[i]);
-        return;
-    }
-    // Each row's columns take the sums over the V that it attends.
-#pragma unroll 1
-    for (int c = 0; c < HEADS; c += group) {
-        const int seen = __builtin_amdgcn_readlane(len.own, c) - first - 4 * g;         // of positions r and 16 + r
-        const auto pair = [&](int r) { return (r < seen ? 0xFFFFu : 0u) | (r + 1 < seen ? 0xFFFF0000u : 0u); };
-        const uint4 mask = make_uint4(pair(0), pair(2), pair(16), pair(18));
-        const bool mine = (lane & 15) >= c && (lane & 15) < c + group;
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-            const uint4 v = operand(i);
-            const f32x4 o = add(make_uint4(v.x & mask.x, v.y & mask.y, v.z & mask.z, v.w & mask.w), st.o[i]);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) st.o[i][r] = mine ? o[r] : st.o[i][r];
-            __builtin_amdgcn_sched_barrier(0);      // one at a time: this is rare, and its registers are not to be had
-        }
+        for (int b = 0; b < H::PARTS; ++b) st.o[i] = H::mfma(__builtin_bit_cast(typename H::vec, v), p[b], st.o[i]);
     }
 }
 
@@ -401,10 +401,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_kernel(AttendArgs a) {
         tile_load<D, NT>(a, kvh, tile, pages, lane, ta);
         pages = tile_pages(a, table, tile + step);
         if constexpr (D > 128 || (ROWS && D > 96)) {
-            // A tile is 128 registers (D = 128: 64, beside what the rows' separation takes): one at a time, two waves a
-            // SIMD to fill each other's waits.
+            // A tile is 128 registers (D = 128, rows of one table: 64): one at a time, two waves a SIMD or three to fill
+            // each other's waits.
             for (;;) {
-                tile_attend<T, D, ROWS>(q, ta, tile * TILE, len, lane, a.group, st);
+                tile_attend<T, D, ROWS>(q, ta, tile * TILE, len, lane, st);
                 tile += step;
                 if (tile >= end) break;
                 tile_load<D, NT>(a, kvh, tile, pages, lane, ta);
@@ -416,12 +416,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attend_kernel(AttendArgs a) {
                 const int next = tile + step;
                 if (next < end) tile_load<D, NT>(a, kvh, next, pages, lane, tb);
                 pages = tile_pages(a, table, next + step);
-                tile_attend<T, D, ROWS>(q, ta, tile * TILE, len, lane, a.group, st);
+                tile_attend<T, D, ROWS>(q, ta, tile * TILE, len, lane, st);
                 if (next >= end) break;
                 tile = next + step;
                 if (tile < end) tile_load<D, NT>(a, kvh, tile, pages, lane, ta);
                 pages = tile_pages(a, table, tile + step);
-                tile_attend<T, D, ROWS>(q, tb, next * TILE, len, lane, a.group, st);
+                tile_attend<T, D, ROWS>(q, tb, next * TILE, len, lane, st);
                 if (tile >= end) break;
             }
         }

@@ -52,3 +52,30 @@ def test_attention_largest_finite_values_behind_a_rise(gpu, dtype, rise):
     k, v = c.arrays()
     want, bound = S.attention(q.reshape(1, 2, d), k, v, c.table, c.pos, d ** -0.5)
     assert (np.abs(got.reshape(1, 2, d) - want).max(-1) <= bound).all(), got[0, :2]
+
+
+# ------------------------------------------ V that is no number, rows of one table
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d,heads,kv_heads", [(64, 8, 2), (96, 3, 1), (128, 4, 2), (256, 2, 1)])
+def test_attention_rows_of_one_table_nonfinite_values(gpu, dtype, d, heads, kv_heads):
+    """NaN and infinities in V, several of a tile: each reaches its own dimension of the rows that attend it, and the
+    bits of everything else stay. Rows out of order, empty ones and one past the table among them; a page is absent."""
+    c = Cached([150], kv_heads, d, 16, dtype)
+    c.table[0, 2] = -1                                           # positions 32 .. 47
+    pos = np.array([70, 3, -1, 149, 64, 65, 66, 2 ** 31 - 1, 31, 100, 0, 40, 71, 72], np.int32)
+    q = dev(np.random.default_rng(d).standard_normal((len(pos), heads * d)).astype(np.float32))
+    args = (dev(c.table).expand(len(pos), -1), dev(pos))
+    c.table[0, 10:] = -1
+    clean = host(gpu.paged_attention(q, c.k, c.v, *args)).reshape(len(pos), heads, d)
+    bad = np.zeros(clean.shape, bool)
+    places = [(65, 0, 0, np.nan), (66, 0, 0, np.inf), (66, kv_heads - 1, d - 1, -np.inf), (3, 0, 5, np.inf), (71, 0, 17, np.nan)]
+    for at, h, dim, value in places:
+        c.v[int(c.table[0, at // 16]), h, at % 16, dim] = value
+        per = heads // kv_heads
+        bad[pos >= at, h * per:(h + 1) * per, dim] = True
+    got = host(gpu.paged_attention(q, c.k, c.v, *args)).reshape(len(pos), heads, d)
+    attended = pos < 150                                         # the one past the table meets slots never filled
+    assert np.array_equal(np.isfinite(got[attended]), ~bad[attended])
+    assert np.array_equal(got[attended][~bad[attended]], clean[attended][~bad[attended]])
