@@ -75,11 +75,12 @@ int w4a8_rope_append(const float *qkv, int heads, const w4a8_kv_cache *cache, co
  * row's own token has been appended): out[i][h] = sum_j p_j v_j, p the softmax
  * over j of scale * (q[i][h] . k_j), query head h reading KV head
  * h / (heads / kv_heads). q, out: float32 [m][heads * head_dim], 16-byte
- * aligned, out no part of q. Scores, softmax and sums are float32; q and p meet
- * the cache's 16-bit values split into as many 16-bit parts as hold 22 bits or
- * more of them. A row without a position left (empty, or all its pages absent)
- * gives zeros. Finite K and V give finite outputs, V up to the type's largest
- * included (for which bf16 weights under 2^-88 of a row's largest are dropped).
+ * aligned, out no part of q. Scores, softmax and sums are float32. q and p meet
+ * the cache's 16-bit values in 16-bit parts: q holds 22 bits, or steps of 2^-38
+ * of its head's largest |q| where those are coarser (fp16); p holds 22 bits at
+ * any size (bf16: down to 2^-64 of the row's largest, and none under 2^-88). A
+ * row without a position left (empty, or all its pages absent) gives zeros.
+ * Finite K and V give finite outputs, V up to the type's largest included.
  * Infinite K or V at a position attended gives non-finite outputs.
  * workspace: w4a8_paged_attention_workspace_bytes of device memory, 16-byte
  * aligned, its contents without meaning between calls; calls that may overlap

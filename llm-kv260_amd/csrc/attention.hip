@@ -19,7 +19,9 @@
 //    dimensions of eight positions has: one v_perm a register.
 //  * The cache's values are exact in the products, q and p are float32: each is
 //    split into 16-bit parts whose sum holds 22 bits (fp16: 2 parts) or 24
-//    (bf16: 3), one MFMA a part.
+//    (bf16: 3), one MFMA a part. fp16's exponents end 30 powers of two under a
+//    head's largest |q|, and what lies 17 under it has fewer bits; p keeps its
+//    bits at any size (Half).
 //  * ref moves only when a score passes it by 2^8 (a vote; about once in a
 //    row), so the loop has no exchange between lanes and no rescaling.
 //  * A row's positions are split over workgroups where rows and heads alone do
@@ -41,7 +43,6 @@ constexpr int TILE = 32;          // positions a wave takes at a time
 constexpr int WAVES = 4;
 constexpr int HEADS = 16;         // columns: query heads a workgroup takes, of a row or of several
 constexpr int MAX_SPLITS = 256;   // of a row: the join gives each a thread
-constexpr float P_LAZY = 8.0f;    // scores may pass ref by it before ref moves
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -56,9 +57,17 @@ struct Half<f16_t> {
     static constexpr int PARTS = 2;
     static constexpr uint32_t EXPONENT = 0x7C00;
     static constexpr bool SCALED = true;    // q is brought to fp16's range by a power of two a head
-    // log2 of what stands for a p of 1 at ref: 2^(7 + P_LAZY) is below fp16's largest, and the low part's 2^-25 under
-    // 2^-32 of the largest p.
-    static __device__ __forceinline__ float unit(int) { return 7.0f; }
+    static constexpr float LAZY = 4.0f;     // scores may pass ref by it before ref moves
+    // log2 of what stands for a p of 1 at ref: p is at most 2^15, half of fp16's range.
+    static __device__ __forceinline__ float unit(int) { return 15.0f - LAZY; }
+    // p's parts: its rounding to fp16, and 2^12 times what that leaves (2^3 at most), whose products are scaled back in
+    // float32. Together they hold 22 bits down to fp16's least normal, 2^-14, which is 2^-25 of a p at ref: a band. What
+    // is under it is taken 2^29 times as large in a band of its own, and so on to float32's least. (An unscaled low part
+    // would lose bits from 2^-10 of the largest p on, and hold nothing under 2^-32.) The scale costs D / 4 multiply-adds a
+    // lane and tile and the wait for the low products: one to three percent (two rows of 131072 of D 64 87.6 -> 88.6 us, 24
+    // of 640 15.4 -> 15.6), a row of 300 5.5 -> 5.9; rows whose scores all lie 17 nats apart, a second band in every tile,
+    // 97 us of the 87.6.
+    static constexpr float LOW = 0x1p12f, LEAST = 0x1p-14f, BAND = 0x1p29f;
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -69,10 +78,11 @@ struct Half<bf16_t> {
     static constexpr int PARTS = 3;
     static constexpr uint32_t EXPONENT = 0x7F80;
     static constexpr bool SCALED = false;
+    static constexpr float LAZY = 8.0f;
     // V may be as large as a float32: p is at most 1 / len, so that no sum of p v passes the largest v. What is left of
     // float32's range below holds p to 22 bits down to 2^-64 of the row's largest, and none under 2^-88 (len = 2^30).
     static __device__ __forceinline__ float unit(int len) {
-        return -P_LAZY - (float)(len > 1 ? 32 - __builtin_clz((unsigned)(len - 1)) : 0);
+        return -LAZY - (float)(len > 1 ? 32 - __builtin_clz((unsigned)(len - 1)) : 0);
     }
     static __device__ __forceinline__ f32x4 mfma(vec a, vec b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -92,6 +102,33 @@ __device__ __forceinline__ void split8(const float (&x)[8], typename Half<T>::ve
             out[p][j] = (T)rest[j];
             rest[j] -= (float)out[p][j];
         }
+}
+
+// fp16's two parts of p, the second scaled (Half::LOW).
+template <class T>
+__device__ __forceinline__ void split_scaled(const float (&p)[8], typename Half<T>::vec (&out)[2]) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        out[0][j] = (T)p[j];
+        out[1][j] = (T)((p[j] - (float)out[0][j]) * Half<T>::LOW);
+    }
+}
+
+// Whether any lane's p has values under its band (Half::LEAST; 0 is none, NaN stays in p): if so they go from p to
+// `under`, scaled to the next.
+template <class T>
+__device__ __forceinline__ bool next_band(float (&p)[8], float (&under)[8]) {
+    uint32_t least = ~0u;               // of the bits less one: 0 comes last
+#pragma unroll
+    for (int j = 0; j < 8; ++j) least = min(least, __float_as_uint(p[j]) - 1);
+    if (__builtin_amdgcn_ballot_w64(least < __float_as_uint(Half<T>::LEAST) - 1) == 0) return false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const bool small = p[j] < Half<T>::LEAST;
+        under[j] = small ? p[j] * Half<T>::BAND : 0.0f;
+        p[j] = small ? 0.0f : p[j];
+    }
+    return true;
 }
 
 struct AttendArgs {
@@ -230,9 +267,10 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[4 * h + r] = H::SCALED ? __builtin_amdgcn_ldexpf(acc[h][r], q.exp) : acc[h][r];
     // Dimension n D / 16 + i of the lane's eight positions.
+    uint32_t lows = 0x05040100u, highs = 0x07060302u;
     const auto operand = [&](int i) {
         const auto word = [&](int j) { return t.v[j][i / 8][(i % 8) / 2]; };
-        const uint32_t sel = i & 1 ? 0x07060302u : 0x05040100u;
+        const uint32_t sel = i & 1 ? highs : lows;
         return make_uint4(__builtin_amdgcn_perm(word(1), word(0), sel), __builtin_amdgcn_perm(word(3), word(2), sel),
                           __builtin_amdgcn_perm(word(5), word(4), sel), __builtin_amdgcn_perm(word(7), word(6), sel));
     };
@@ -286,7 +324,7 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
     float top = s[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
-    if (__builtin_amdgcn_ballot_w64(top > st.ref + P_LAZY) != 0) {
+    if (__builtin_amdgcn_ballot_w64(top > st.ref + H::LAZY) != 0) {
         top = fmaxf(top, __shfl_xor(top, 16));
         top = fmaxf(top, __shfl_xor(top, 32));
         const float ref = fmaxf(st.ref, top);
@@ -301,12 +339,53 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
     for (int j = 0; j < 8; ++j) s[j] = __builtin_amdgcn_exp2f(s[j] - base);
     st.sum += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
     typename H::vec p[H::PARTS];
-    split8<T>(s, p);
+    if constexpr (!H::SCALED) {
+        split8<T>(s, p);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-        const uint4 v = operand(i);
+        for (int i = 0; i < D / 16; ++i) {
+            const auto v = __builtin_bit_cast(typename H::vec, operand(i));
 #pragma unroll
-        for (int b = 0; b < H::PARTS; ++b) st.o[i] = H::mfma(__builtin_bit_cast(typename H::vec, v), p[b], st.o[i]);
+            for (int b = 0; b < H::PARTS; ++b) st.o[i] = H::mfma(v, p[b], st.o[i]);
+        }
+    } else {
+        const auto add_scaled = [](f32x4 x, float f, f32x4 &o) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = fmaf(x[r], f, o[r]);
+        };
+        float under[8], band = 1.0f;
+        bool more = next_band<T>(s, under);
+        split_scaled<T>(s, p);
+        constexpr int AT_ONCE = D > 128 ? 2 : 4;         // low products on their way: registers
+#pragma unroll
+        for (int i = 0; i < D / 16; i += AT_ONCE) {
+            f32x4 low[AT_ONCE];
+#pragma unroll
+            for (int j = 0; j < AT_ONCE && i + j < D / 16; ++j) {
+                const auto v = __builtin_bit_cast(typename H::vec, operand(i + j));
+                low[j] = H::mfma(v, p[1], f32x4{});
+                st.o[i + j] = H::mfma(v, p[0], st.o[i + j]);
+            }
+#pragma unroll
+            for (int j = 0; j < AT_ONCE && i + j < D / 16; ++j) add_scaled(low[j], 1.0f / H::LOW, st.o[i + j]);
+        }
+        // The bands under the first, one dimension tile after the other: few tiles have any.
+        while (__builtin_expect(more, false)) {
+            float now[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) now[j] = under[j];
+            more = next_band<T>(now, under);
+            split_scaled<T>(now, p);
+            band *= 1.0f / H::BAND;
+            // Other constants, as far as the compiler knows: it would keep all of V's operands from band to band. (Not
+            // volatile, which would count as a store and make the page table's scalar loads vector ones.)
+            __asm__("" : "+s"(lows), "+s"(highs));
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+                const auto v = __builtin_bit_cast(typename H::vec, operand(i));
+                add_scaled(H::mfma(v, p[0], f32x4{}), band, st.o[i]);
+                add_scaled(H::mfma(v, p[1], f32x4{}), band / H::LOW, st.o[i]);
+            }
+        }
     }
 }
 

@@ -2,6 +2,8 @@
 
 from __future__ import annotations
 
+import math
+
 import numpy as np
 import pytest
 
@@ -79,3 +81,74 @@ def test_attention_rows_of_one_table_nonfinite_values(gpu, dtype, d, heads, kv_h
     attended = pos < 150                                         # the one past the table meets slots never filled
     assert np.array_equal(np.isfinite(got[attended]), ~bad[attended])
     assert np.array_equal(got[attended][~bad[attended]], clean[attended][~bad[attended]])
+
+
+# ---------------------------------------------- weights far below the largest
+
+
+def _one_channel(c, scores, vals):
+    """Keys of one row whose score against q = 8 e_0 at scale 1 / 8 is `scores` exactly, with `vals` [n, d]."""
+    import torch
+    page = c.k.shape[2]
+    at = torch.from_numpy(c.table[0, np.arange(len(scores)) // page].astype(np.int64)).cuda()
+    slot = torch.arange(len(scores), device="cuda") % page
+    c.k[at, :, slot] = 0.0
+    c.k[at, :, slot, 0] = dev(scores)[:, None].to(c.dtype)
+    c.v[at, :, slot] = dev(vals)[:, None].to(c.dtype)
+
+
+def _check_relative(gpu, c, scores, rows, heads=2):
+    """Every output within its own relative bound: V is nowhere negative, so nothing cancels.
+
+    A score of at most `far` nats: the factor scale log2 e and its product with q are rounded (2^-24 each), q is held to
+    22 bits or more, the products' sum and the distance from the reference are rounded (2^-24 each): far 2^-21 nats
+    in all at most, a relative error as large in p. p is an exponential within 2^-22 and held to 2^-22: 2^-21. The sums
+    of p v and of p: n / 32 + 128 roundings each, as step_oracle's bound has them. Weights are held to 2^-88 of the largest
+    at least, each times a V of at most max |V|."""
+    d, n = c.k.shape[-1], len(scores)
+    q = np.zeros((rows, heads, d), np.float32)
+    q[:, :, 0] = 8.0
+    c.pos = np.full(rows, n - 1, np.int32)
+    got = host(gpu.paged_attention(dev(q.reshape(rows, -1)), c.k, c.v, dev(c.table).expand(rows, -1), dev(c.pos),
+                                   scale=0.125)).reshape(rows, heads, d)
+    k, v = c.arrays()
+    want, _ = S.attention(q, k, v, c.table.repeat(rows, 0), c.pos, 0.125)
+    far = float(np.max(np.abs(scores)))
+    tol = 1.01 * far * 2.0 ** -21 + 2.0 ** -20 + 2 * (n / 32 + 128) * 2.0 ** -24
+    rel = (np.abs(got - want) - n * 2.0 ** -88 * np.nanmax(v)) / want
+    assert (want > 0).all() and rel.max() <= tol, (rel.max(), tol)
+
+
+@pytest.mark.parametrize("dtype,nats", [("float16", (14, 18, 20, 25, 33, 45, 60, 80)), ("bfloat16", (14, 20, 33, 45))])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("n,at", [(20, 0), (20, 11), (4003, 0), (4003, 4002), (4003, 1777)])
+def test_attention_sink(gpu, dtype, nats, d, n, at):
+    """One key that takes nearly all the weight, its V zero: the output is the rest's, however small their weights."""
+    rng = np.random.default_rng(n + at)
+    c = Cached([n], 1, d, 64, dtype)
+    vals = (0.5 + rng.random((n, d))).astype(np.float32)
+    vals[at] = 0.0
+    for far in nats:
+        scores = np.zeros(n, np.float32)
+        scores[at] = far
+        _one_channel(c, scores, vals)
+        for rows in (1, 3):                                     # alone, and rows of one table
+            _check_relative(gpu, c, scores, rows)
+
+
+@pytest.mark.parametrize("dtype,far", [("float16", 26), ("bfloat16", 44)])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("n", [33, 1500])
+def test_attention_weights_of_every_size(gpu, dtype, far, d, n):
+    """Scores spread over `far` nats, V a power of two that makes up for the weight: every key counts alike."""
+    rng = np.random.default_rng(n)
+    scores = (rng.integers(0, 4 * far + 1, n) / 4).astype(np.float32)
+    scores[rng.integers(n)] = far
+    span = round(far * math.log2(math.e))
+    low = -24 if dtype == "float16" else -20
+    vals = np.exp2(low + np.round((far - scores) * math.log2(math.e)))[:, None] * (1 + rng.integers(0, 2, (n, d)))
+    assert vals.max() <= 65504 or dtype == "bfloat16" and span < 100
+    c = Cached([n], 1, d, 32, dtype)
+    _one_channel(c, scores, vals.astype(np.float32))
+    for rows in (1, 3):
+        _check_relative(gpu, c, scores, rows)
