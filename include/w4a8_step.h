@@ -80,8 +80,11 @@ int w4a8_rope_append(const float *qkv, int heads, const w4a8_kv_cache *cache, co
  * of its head's largest |q| where those are coarser (fp16); p holds 22 bits at
  * any size (bf16: down to 2^-64 of the row's largest, and none under 2^-88). A
  * row without a position left (empty, or all its pages absent) gives zeros.
- * Finite K and V give finite outputs, V up to the type's largest included.
- * Infinite K or V at a position attended gives non-finite outputs.
+ * Finite K and V give finite outputs, V up to the type's largest included, where
+ * the scores are within float32's range. An infinite or NaN K (or a score past
+ * that range) at a position attended makes the outputs of its row's query heads
+ * of that KV head NaN, an infinite or NaN V the outputs of its dimension there
+ * non-finite.
  * workspace: w4a8_paged_attention_workspace_bytes of device memory, 16-byte
  * aligned, its contents without meaning between calls; calls that may overlap
  * need one each. */

@@ -265,7 +265,12 @@ __device__ __forceinline__ void tile_attend(const Query<T, D> &q, Tile<D> &t, in
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[4 * h + r] = H::SCALED ? __builtin_amdgcn_ldexpf(acc[h][r], q.exp) : acc[h][r];
+        for (int r = 0; r < 4; ++r) {
+            s[4 * h + r] = H::SCALED ? __builtin_amdgcn_ldexpf(acc[h][r], q.exp) : acc[h][r];
+            // An infinite K meets q's parts one by one, with either sign: whatever that gives, the output is NaN (it is so
+            // for +inf and NaN), for -inf would drop the position.
+            if (s[4 * h + r] == -INFINITY) s[4 * h + r] = NAN;
+        }
     // Dimension n D / 16 + i of the lane's eight positions.
     uint32_t lows = 0x05040100u, highs = 0x07060302u;
     const auto operand = [&](int i) {

@@ -152,3 +152,33 @@ def test_attention_weights_of_every_size(gpu, dtype, far, d, n):
     _one_channel(c, scores, vals.astype(np.float32))
     for rows in (1, 3):
         _check_relative(gpu, c, scores, rows)
+
+
+# ------------------------------------------------------------------ infinite K
+
+
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+def test_attention_infinite_keys(gpu, dtype, d, value):
+    """An infinite K at a position attended gives NaN in its row and KV head, whatever q's sign and bits there, and
+    leaves the others' bits alone."""
+    import torch
+    c = Cached([100, 100, 1500], 2, d, 32, dtype)
+    heads, per = 16, 8
+    g = torch.Generator(device="cuda").manual_seed(d)
+    q = torch.randn((3, heads, d), generator=g, device="cuda")
+    q[:, 8, 7], q[:, 9, 7], q[:, 10, 7], q[:, 11, 7] = 0.0, 1.0, -1.0, 2.0 ** -12
+    q = q.view(3, -1)
+    args = (dev(c.table), dev(c.pos))
+    clean = host(gpu.paged_attention(q, c.k, c.v, *args)).reshape(3, heads, d)
+    c.k[int(c.table[0, 1]), 1, 9, 7] = value
+    c.k[int(c.table[2, 40]), 1, 3, 7] = value
+    got = host(gpu.paged_attention(q, c.k, c.v, *args)).reshape(3, heads, d)
+    assert np.isnan(got[[0, 2], per:]).all()
+    assert np.array_equal(got[1], clean[1]) and np.array_equal(got[:, :per], clean[:, :per])
+    # Rows of one table: those that attend the position, and no row before it.
+    pos = torch.arange(30, 60, dtype=torch.int32, device="cuda")         # the key's is 41
+    q = torch.randn((30, heads * d), generator=g, device="cuda")
+    got = host(gpu.paged_attention(q, c.k, c.v, args[0][:1].expand(30, -1), pos)).reshape(30, heads, d)
+    assert np.isnan(got[11:, per:]).all() and np.isfinite(got[:11]).all() and np.isfinite(got[:, :per]).all()
