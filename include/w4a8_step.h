@@ -63,10 +63,11 @@ typedef struct w4a8_kv_rows {
  * it. q_out: float32 [m][heads * head_dim], 16-byte aligned, may be no part of
  * qkv; zeros for an empty row, whose cache entries are left as they are.
  * inv_freq: float32 [rope_dim / 2], the angle of pair i being pos * inv_freq[i]
- * radians (reduced in float64); rope_dim even, 2 .. head_dim, dimensions past
- * it pass unrotated. Pairs are (i, i + rope_dim / 2), or (2i, 2i + 1) with
- * interleaved (GGUF's Llama order, board/tp/tp_llama.cpp:528-705). Two rows of
- * one call must not share a page and position: either's values may stand.
+ * radians (sine and cosine within 2^-23, up to 2^40 of them); rope_dim even, 2 ..
+ * head_dim, dimensions past it pass unrotated. Pairs are (i, i + rope_dim / 2), or
+ * (2i, 2i + 1) with interleaved (GGUF's Llama order, board/tp/tp_llama.cpp:528-705).
+ * Two rows of one call must not share a page and position: either's values may
+ * stand.
  * heads a multiple of kv_heads, m * heads at most 2^22. */
 int w4a8_rope_append(const float *qkv, int heads, const w4a8_kv_cache *cache, const w4a8_kv_rows *rows,
                      const float *inv_freq, int rope_dim, int interleaved, float *q_out, void *stream);

@@ -19,16 +19,17 @@ namespace w4a8 {
 
 namespace {
 
-// sin and cos of pos * freq, within 2^-23. The product of a 31-bit integer and
-// a float32 is exact in float64 to 2^-53 of it, and so is what is left of it
-// by the nearest multiple of pi / 2 (to 2^-22 of an ulp at 2^30 radians): far
-// positions are as exact as near ones. Then, |r| <= pi / 4, the series of both
-// in float32, to r^9 and r^10 (the next terms are under 2^-29), what float32
-// left of r carried as `lo` through the first-order terms.
+// sin and cos of pos * freq, within 2^-23 up to 2^40 radians. The product of a
+// 31-bit integer and a float32 may take 55 bits: it is held as a float64 and what
+// that leaves. Of both, what is left by the nearest multiple of pi / 2 (two
+// float64, so to 2^-69 there) is taken: far positions are as exact as near ones.
+// Then, |r| <= pi / 4, the series of both in float32, to r^9 and r^10 (the next
+// terms are under 2^-29), what float32 left of r carried as `lo` through the
+// first-order terms.
 __device__ __forceinline__ void rope_angle(int pos, float freq, float &s, float &c) {
-    const double a = (double)pos * (double)freq;
+    const double a = (double)pos * (double)freq, rest = fma((double)pos, (double)freq, -a);
     const double n = rint(a * 0.63661977236758134308);           // 2 / pi
-    const double r = fma(n, -6.1232339957367660359e-17, fma(n, -1.5707963267948965580, a));
+    const double r = fma(n, -6.1232339957367660359e-17, fma(n, -1.5707963267948965580, a)) + rest;
     const float hi = (float)r, lo = (float)(r - (double)hi);
     const float z = hi * hi;
     float p = fmaf(z, 1.0f / 362880, -1.0f / 5040);

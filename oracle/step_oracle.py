@@ -4,8 +4,33 @@ rope and the cache append, paged attention, the residual norms, the sampler's dr
 from __future__ import annotations
 
 import math
+from fractions import Fraction
 
 import numpy as np
+
+
+def _arctan_of_inverse(n: int, one: int) -> int:
+    """arctan(1 / n) one, by its series in integers."""
+    total, power, i = 0, one // n, 1
+    while power:
+        total += power // i if i % 4 == 1 else -(power // i)
+        power //= n * n
+        i += 2
+    return total
+
+
+# 2 pi to 300 bits (Machin's formula).
+_TURN = Fraction(2 * (16 * _arctan_of_inverse(5, 1 << 320) - 4 * _arctan_of_inverse(239, 1 << 320)), 1 << 320)
+
+
+def angles(pos: np.ndarray, freq: float) -> np.ndarray:
+    """pos * freq radians: the float64 product where it is exact (24 bits of freq times 29 of pos), else what is left of
+    the exact product by the nearest multiple of 2 pi."""
+    out = pos.astype(np.float64) * float(freq)
+    for i in np.nonzero(pos >= 2 ** 29)[0]:
+        a = Fraction(int(pos[i])) * Fraction(float(freq))
+        out[i] = float(a - round(a / _TURN) * _TURN)
+    return out
 
 
 def rope(x: np.ndarray, pos: np.ndarray, inv_freq: np.ndarray, interleaved: bool) -> np.ndarray:
@@ -15,7 +40,7 @@ def rope(x: np.ndarray, pos: np.ndarray, inv_freq: np.ndarray, interleaved: bool
     half = inv_freq.size
     for i in range(half):
         a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
-        angle = pos.astype(np.float64) * float(inv_freq[i])
+        angle = angles(pos, inv_freq[i])
         c, s = np.cos(angle)[:, None], np.sin(angle)[:, None]
         y[:, :, a] = x[:, :, a] * c - x[:, :, b] * s
         y[:, :, b] = x[:, :, b] * c + x[:, :, a] * s

@@ -787,3 +787,24 @@ def test_decode_steps(gpu):
         assert token == S.sample(host(logits), host(u)[step], 0.8, 40, 0.95)
         drawn.append(token)
     assert len(set(drawn)) > 3
+
+
+# ----------------------------------------------------------- far positions
+
+
+@pytest.mark.parametrize("first,freqs", [(0, (0.0, 1.0)), (2 ** 29, (0.5, 1.0)), (2 ** 31 - 4000, (0.5, 1.0)),
+                                         (2 ** 31 - 4000, (1e-6, 1e-2)), (2 ** 31 - 4000, (1.0, 512.0))])
+def test_append_angles(gpu, first, freqs):
+    """Sine and cosine themselves, of unit pairs: within 2^-23 of the exact angle's at every position and frequency of
+    up to 2^40 radians. The positions lie past the table: nothing is stored."""
+    m, d = 2000, 64
+    rng = np.random.default_rng(first % 1000 + 1)
+    inv = rng.uniform(*freqs, d // 2).astype(np.float32)
+    pos = np.sort(rng.integers(first, min(first + 200000, 2 ** 31), m)).astype(np.int32)
+    c = Cached([16], 1, d, 16, "float16")
+    qkv = np.zeros((m, 3 * d), np.float32)
+    qkv[:, : d // 2] = 1.0
+    got = host(gpu.rope_append(dev(qkv), c.k, c.v, dev(np.full((1, 1), -1, np.int32)).expand(m, -1), dev(pos), dev(inv)))
+    angle = np.stack([S.angles(pos, f) for f in inv], 1)
+    err = np.abs(got - np.concatenate([np.cos(angle), np.sin(angle)], 1))
+    assert err.max() <= 2.0 ** -23, err.max() * 2.0 ** 23

@@ -194,3 +194,14 @@ def test_oracle_sample_known_answers():
     assert [S.sample(l, u, top_p=0.45) for u in (0.49, 0.51)] == [1, 2]
     assert S.sample(l, 0.99, top_p=0.39) == 1 and S.sample(l, 0.99, min_p=0.5) == 2 and S.sample(l, 0.99, temperature=0) == 1
     assert S.sample([-np.inf, np.nan], 0.5) == -1
+
+
+def test_oracle_angles_of_far_positions():
+    """Against the math library's own reduction: of an integer, and of an integer and a small angle apart."""
+    pos = np.array([0, 5, 2 ** 29 - 1, 2 ** 29 + 1, 10 ** 9 + 7, 2 ** 31 - 1])
+    got = S.angles(pos, np.float32(1.0))
+    assert np.allclose(np.sin(got), np.sin(pos.astype(np.float64)), rtol=0, atol=1e-14)
+    assert np.abs(got[3:]).max() <= np.pi + 1e-12
+    small = pos * 2.0 ** -23
+    want = np.sin(pos.astype(np.float64)) * np.cos(small) + np.cos(pos.astype(np.float64)) * np.sin(small)
+    assert np.allclose(np.sin(S.angles(pos, np.float32(1 + 2.0 ** -23))), want, rtol=0, atol=1e-13)
