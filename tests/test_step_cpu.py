@@ -205,3 +205,19 @@ def test_oracle_angles_of_far_positions():
     small = pos * 2.0 ** -23
     want = np.sin(pos.astype(np.float64)) * np.cos(small) + np.cos(pos.astype(np.float64)) * np.sin(small)
     assert np.allclose(np.sin(S.angles(pos, np.float32(1 + 2.0 ** -23))), want, rtol=0, atol=1e-13)
+
+
+def test_sample_workspace_is_checked():
+    """Of rows in slices, the only ones with a workspace."""
+    L = kv.lib()
+    s = kv.Sampling(None, None, None, None, 1.0, 0, 1.0, 0.0)
+    need = L.w4a8_sample_workspace_bytes(3, 20000)
+    assert need > 0 and L.w4a8_sample_workspace_bytes(3, 5000) == 0
+
+    def call(ws=A[3], size=need):
+        return L.w4a8_sample(A[0], 20000, 3, 20000, A[1], ctypes.byref(s), A[2], ws, size, None)
+
+    assert call(ws=None) == -1
+    assert call(size=need - 1) == call(size=0) == -2
+    assert call(ws=A[3] + 8) == -3
+    assert call(ws=A[0]) == call(ws=A[1]) == call(ws=A[2]) == -2
