@@ -48,7 +48,9 @@ typedef struct w4a8_kv_cache {
  * share one table row: the tokens of a prompt, or drafted ones, whose attention
  * then reads the cache once for several of them. An entry outside [0, pages) is
  * an absent page: nothing is stored for its positions, and attention takes them
- * as masked; so it does positions from table_pages * page_size on. */
+ * as masked; so it does positions from table_pages * page_size on. How rows are
+ * split over the GPU goes by table_pages: a table no wider than its longest row
+ * needs is the fastest. */
 typedef struct w4a8_kv_rows {
     const int32_t *table;
     int64_t table_stride;   /* entries; 0 or table_pages .. 2^30 */

@@ -22,14 +22,15 @@
 //    (bf16: 3), one MFMA a part. fp16's exponents end 30 powers of two under a
 //    head's largest |q|, and what lies 17 under it has fewer bits; p keeps its
 //    bits at any size (Half).
-//  * ref moves only when a score passes it by 2^8 (a vote; about once in a
-//    row), so the loop has no exchange between lanes and no rescaling.
+//  * ref moves only when a score passes it by some powers of two (Half::LAZY; a
+//    vote; about once in a row), so the loop has no exchange between lanes and no
+//    rescaling.
 //  * A row's positions are split over workgroups where rows and heads alone do
 //    not fill the GPU, and the parts joined by a second launch.
 //
-// Measured, 32 heads over 8: two rows of 131072 (D 64) 88 us, 6.1 TB/s; 64 rows
-// of up to 8192 (D 128, ragged) 203 us, 5.6 TB/s; a row of 8192 9.9 us; a row
-// of 300 (D 64) 5.5 us, of which the memory's share is under one: the launch,
+// Measured, 32 heads over 8: two rows of 131072 (D 64, fp16) 88 us, 6.1 TB/s; 64
+// rows of up to 8192 (D 128, bf16, ragged) 196 us, 5.8 TB/s; a row of 8192 (D 64,
+// fp16) 9.6 us; a row of 300 (D 64, fp16) 6.0 us, of which the memory's share is under one: the launch,
 // three dependent loads (table, K, V) and the waves' join.
 #include "../../include/w4a8_step.h"
 #include "kernels.h"
@@ -621,20 +622,23 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
         sum == 0.0f ? make_float4(0.0f, 0.0f, 0.0f, 0.0f) : make_float4(o.x / sum, o.y / sum, o.z / sum, o.w / sum);
 }
 
-// Rows that a workgroup takes together: those of one table, as many as fill its columns. 32 heads over 8, in us, alone
-// and together: 128 rows of a prompt (D 64) 9.2 and 9.8, 512 rows 35 and 16, 2048 rows 394 and 117; D 128: 512 rows 61
-// and 25, 2048 rows 711 and 197.
+// Rows that a workgroup takes together: those of one table, as many as fill its columns. 32 heads over 8, fp16, in us,
+// alone and together: a prompt of 16 rows (D 64) 4.1 and 4.8, 128 rows 7.4 and 5.1, 512 rows 36 and 14.6, 2048 rows 368
+// and 104; D 128: 512 rows 57 and 20.5, 2048 rows 685 and 170. Bound by the reads from the caches, 10 TB/s at 2048 rows:
+// every four rows read all of K and V. Rows drafted behind 32768 (D 64): two 26 and 18, eight 70 and 21; behind 2048 two
+// 7.4 and 7.7, eight 10.4 and 8.2.
 int attend_rows_each(int group, const w4a8_kv_rows &r) {
     return r.table_stride == 0 && r.m > 1 && group <= HEADS / 2 ? HEADS / group : 1;
 }
 
-// Splits of a row, by the length that its table allows and what rows and heads leave of the GPU (groups of them; a
+// Splits of a row, by the length that its table allows (all that the host knows of it: a row of 300 takes 6.1 us with a
+// table of its own width and 8.0 with one of 8192 or 131072, eight of up to 2048 14.1, 14.0 and 28.1) and what rows and heads leave of the GPU (groups of them; a
 // round is the 128 positions that a workgroup's waves take at once). Measured, in us:
-//  * up to three rounds, one: the join costs 2.5, a round 1 (300 positions 5.5 against 7.0 in three splits; 512
-//    positions, four rounds, 8.6 whole and 7.9 split).
+//  * up to three rounds, one: the join costs 2.5, a round 1 (300 positions, D 64, 6.1 against 7.2 in three splits; 512
+//    positions, four rounds, D 128, 8.9 whole and 8.1 split; D 64 6.8 and 7.2).
 //  * to eight rounds also where the groups alone give three quarters of the compute units one: no join, and the rows
-//    need not be read in turn (24 rows of 640, 192 groups: 14.1 whole, 19.0 in three; 32 of 1024 at most, ragged: 21.3
-//    and 24.6 in two; 16 of 1024, 128 groups: 19.9 and 17.3 in four).
+//    need not be read in turn (24 rows of 640, 192 groups: 14.3 whole, 19.2 in three; 32 of 1024 at most, ragged: 20.0
+//    and 23.9 in two; 16 of 1024, 128 groups: 20.2 and 17.8 in four).
 //  * else to 512 workgroups, two a compute unit, a round each at least (one row of 8192: 9.9 with 64 splits, 10.9 with
 //    16; sixteen of 2048: 31.7 with 512 workgroups, 32.4 with 1024, 36.6 with 2048; 128 rows of 1024: 98.5 whole,
 //    109.6 in two).

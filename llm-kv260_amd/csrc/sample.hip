@@ -25,11 +25,12 @@
 // need be. A row of one slice does all of it in the third launch's workgroup,
 // the only one then.
 //
-// Measured, 128256 logits: a row with top-k 40 16.2 us (2.7 + 5.1 + 8.4), with
-// top-p 0.95 19.6, 64 rows of all kinds 44.7 (0.7 TB/s). One pass over the
+// Measured, 128256 logits: a row with top-k 40 16.1 us, with top-p 0.95 19.9, 64
+// rows of all kinds 43.7 (0.75 TB/s); the launches of the first 2.9 + 5.3 + 9.2 in
+// a profile, which adds a little to each, of the last 7.0 + 16.8 + 22.3. One pass over the
 // bytes would take 0.1 and 6.9 us: few rows are bound by three launches that
 // wait for each other and the third's prefix sums and list, many by the second's
-// float64 exponentials and LDS atomics (15) and the third's issue (18).
+// float64 exponentials and LDS atomics and the third's issue.
 #include "../../include/w4a8_step.h"
 #include "kernels.h"
 
@@ -704,7 +705,9 @@ __global__ __launch_bounds__(ALONE ? ALONE_THREADS : ROW_THREADS) void row_kerne
 // 28.9 us whole, 35.9 in two; of 64000 46.9 and 54.7), and where it is done before the three launches of the slices:
 // a workgroup takes n logits in the time in which all take 200 n, plus what the launches cost, that of some 1.9
 // million (one row of 9000 15.3 whole and 16.1 sliced, 17.8 and 15.9 of 16000; 90 rows of 16000 18.9 and 21.7, 64 of
-// 32000 27.0 and 23.5, 128 of 32000 27.8 and 28.2).
+// 32000 27.0 and 23.5, 128 of 32000 27.8 and 28.2). Past 170 rows the rule looks at neither the vocabulary nor the CUs: a
+// workgroup fills one, so up to 256 rows of 128256 are faster whole (256: 110 and 123 in three), 300 are not (177 whole,
+// 154 in two, 142 in three), 512 are again (207 and 220).
 int sample_slices(int m, int n) {
     if (m > 170 || (int64_t)n * (200 - m) <= 1900000) return 1;
     const int most = 512 / m < MAX_SLICES ? 512 / m : MAX_SLICES;
