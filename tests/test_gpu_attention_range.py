@@ -55,6 +55,19 @@ def test_attention_largest_finite_values_behind_a_rise(gpu, dtype, rise):
     want, bound = S.attention(q.reshape(1, 2, d), k, v, c.table, c.pos, d ** -0.5)
     assert (np.abs(got.reshape(1, 2, d) - want).max(-1) <= bound).all(), got[0, :2]
 
+@pytest.mark.parametrize("dtype,exponents", [("float16", (0, -14, -24)), ("bfloat16", (0, -60, -100, -115, -126))])
+@pytest.mark.parametrize("n", [1, 300, 5000])
+def test_attention_smallest_values(gpu, dtype, exponents, n):
+    """Equal scores and one power of two in V: the output is that, exactly (every product p v is a power of two over
+    2^-149, every sum of them and of p a count of them)."""
+    c = Cached([n], 1, 64, 64, dtype)
+    live = ~np.isnan(host(c.v.float()))
+    for e in exponents:
+        for t, value in ((c.k, 0.0), (c.v, 2.0 ** e)):
+            t[dev(live)] = value
+        got = host(gpu.paged_attention(dev(np.ones((1, 128), np.float32)), c.k, c.v, dev(c.table), dev(c.pos)))
+        assert (got == 2.0 ** e).all(), (e, got[0, :2])
+
 
 # ------------------------------------------ V that is no number, rows of one table
 
