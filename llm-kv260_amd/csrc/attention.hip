@@ -30,8 +30,8 @@
 //
 // Measured, 32 heads over 8: two rows of 131072 (D 64, fp16) 88 us, 6.1 TB/s; 64
 // rows of up to 8192 (D 128, bf16, ragged) 196 us, 5.8 TB/s; a row of 8192 (D 64,
-// fp16) 9.6 us; a row of 300 (D 64, fp16) 6.0 us, of which the memory's share is under one: the launch,
-// three dependent loads (table, K, V) and the waves' join.
+// fp16) 9.6 us; a row of 300 (D 64, fp16) 6.0 us, of which the memory's share is
+// under one: the launch, three dependent loads (table, K, V) and the waves' join.
 #include "../../include/w4a8_step.h"
 #include "kernels.h"
 #include "kv_device.h"
@@ -632,8 +632,9 @@ int attend_rows_each(int group, const w4a8_kv_rows &r) {
 }
 
 // Splits of a row, by the length that its table allows (all that the host knows of it: a row of 300 takes 6.1 us with a
-// table of its own width and 8.0 with one of 8192 or 131072, eight of up to 2048 14.1, 14.0 and 28.1) and what rows and heads leave of the GPU (groups of them; a
-// round is the 128 positions that a workgroup's waves take at once). Measured, in us:
+// table of its own width and 8.0 with one of 8192 or 131072, eight of up to 2048 14.1, 14.0 and 28.1) and what rows and
+// heads leave of the GPU (groups of them; a round is the 128 positions that a workgroup's waves take at once). Measured,
+// in us:
 //  * up to three rounds, one: the join costs 2.5, a round 1 (300 positions, D 64, 6.1 against 7.2 in three splits; 512
 //    positions, four rounds, D 128, 8.9 whole and 8.1 split; D 64 6.8 and 7.2).
 //  * to eight rounds also where the groups alone give three quarters of the compute units one: no join, and the rows
